@@ -7,9 +7,9 @@
  * per-pixel entry points, glam-pbr/src/lib.rs is the math).  The reference has no FFI
  * of its own: its boundary is the Vulkan descriptor/push-constant ABI of the two
  * fragment entry points.  Every struct below mirrors one of those wire structs byte
- * for byte (offsets verified against the OpMemberDecorate Offset words of
- * compiled-shaders/normal/fragment_transmission.spv), and every function replaces one
- * step of `record()`; the reference interface each one replaces is cited.
+ * for byte (the #[repr(C)] structs of shared-structs/src/lib.rs; offsets asserted
+ * below), and every function replaces one step of `record()`; the reference interface
+ * each one replaces is cited.
  *
  * Conventions
  *   - plain C, no C++/torch types; device pointers are raw `void*` owned by the caller

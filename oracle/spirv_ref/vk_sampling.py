@@ -1,8 +1,7 @@
 """Vulkan fixed-function image operations in numpy fp32, written from the Vulkan 1.3 specification — NOT from
-oracle/tr_oracle.c.  TEST INFRASTRUCTURE: tools/make_golden_spirv.py answers the SPIR-V interpreter's OpImageSample*
-callbacks and builds the mip chains with THIS module, so that the committed fixtures are "the reference's compiled
-shader binary + the Vulkan specification" and contain no output of the C oracle; tests/test_vk_sampling.py then checks
-that the oracle's samplers agree with it bit for bit.
+oracle/tr_oracle.c.  TEST INFRASTRUCTURE: the image samples and the mip chains in the recorded fixtures (tests/golden/)
+came from THIS module, so they contain no output of the C oracle; tests/test_vk_sampling.py checks that the oracle's
+samplers agree with it bit for bit.
 
 What the specification fixes, and what this module has to choose (stated once, here):
 
@@ -34,7 +33,7 @@ What the specification fixes, and what this module has to choose (stated once, h
 * pow / log2 go through the host's glibc powf / log2f (ctypes), the same library the reference's CPU-side Rust
   (`f32::powf`, `f32::log2` -> the platform libm on Linux) would call; sqrt is numpy's correctly rounded fp32 sqrt.
 
-Scalar entry points (one sample per call, numpy float32 scalars: one IEEE rounding per operation) serve the interpreter;
+Scalar entry points take one sample per call (numpy float32 scalars: one IEEE rounding per operation);
 the chain builders are vectorised over the image with the same per-element operations.
 """
 from __future__ import annotations
@@ -223,7 +222,7 @@ def _levels_of(lod, count: int):
 
 
 def sample_pyramid(levels: Sequence[np.ndarray], u, v, lod) -> np.ndarray:
-    """OpImageSampleExplicitLod of the RGBA16F opaque pyramid through the reference's `clamp_sampler`
+    """An explicit-LOD sample of the RGBA16F opaque pyramid through the reference's `clamp_sampler`
     (src/main.rs:694-705: LINEAR / LINEAR / MIPMAP_MODE_LINEAR, CLAMP_TO_EDGE).  `levels`: (h_l, w_l, 4) float16."""
     d_hi, d_lo, delta = _levels_of(lod, len(levels))
     taps = []
@@ -247,7 +246,7 @@ class _F32View:
 
 
 def sample_lut(rgba8: np.ndarray, u, v) -> np.ndarray:
-    """OpImageSampleImplicitLod of the single-level R8G8B8A8_UNORM GGX LUT through `clamp_sampler`: bilinear."""
+    """An implicit-LOD sample of the single-level R8G8B8A8_UNORM GGX LUT through `clamp_sampler`: bilinear."""
     h, w = rgba8.shape[:2]
     x0, x1, ax = _linear_taps_clamp(u, w)
     y0, y1, by = _linear_taps_clamp(v, h)
@@ -259,7 +258,7 @@ def sample_lut(rgba8: np.ndarray, u, v) -> np.ndarray:
 
 
 def sample_texture(levels: Sequence[np.ndarray], srgb: bool, u, v, duv_dx, duv_dy) -> np.ndarray:
-    """OpImageSampleImplicitLod of a material texture through the reference's `sampler` (src/main.rs:683-692: LINEAR /
+    """An implicit-LOD sample of a material texture through the reference's `sampler` (src/main.rs:683-692: LINEAR /
     LINEAR / MIPMAP_MODE_LINEAR, address modes left at REPEAT): implicit LOD from the quad's uv derivatives."""
     w, h = levels[0].shape[1], levels[0].shape[0]
     mxx, mxy = f32(duv_dx[0]) * f32(w), f32(duv_dx[1]) * f32(h)

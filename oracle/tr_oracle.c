@@ -4,8 +4,7 @@
  * Scalar IEEE fp32 (`real` = float; see tr_oracle.h for the fp64 conditioning twin), one operation per
  * source operation of the reference, in the
  * reference's association order (glam 0.19 scalar Vec3: dot = (x*x'+y*y')+z*z',
- * normalize = v * (1/sqrt(len^2)), lerp = a + (b-a)*t; confirmed against the op order of
- * compiled-shaders/normal/fragment_transmission.spv by oracle/spirv_ref).
+ * normalize = v * (1/sqrt(len^2)), lerp = a + (b-a)*t).
  * Must be compiled with -ffp-contract=off and without -ffast-math.
  */
 #include "tr_oracle.h"
@@ -863,8 +862,7 @@ static o_vec3 calculate_normal(const o_scene* s, o_vec3 interpolated_normal, con
     if (material->textures.normal_map != -1) {
         real smp[4];
         sample_material_texture(s, material->textures.normal_map, uv, d, smp);
-        /* `map_normal * 255.0 / 127.0 - 128.0 / 127.0`: the compiled shader (fragment.spv) multiplies by the
-         * folded constant 255/127 = 2.007874 and subtracts the folded 128/127 */
+        /* map_normal * 255/127 - 128/127, the two quotients of constants formed first */
         o_vec3 map_normal = v3_add_s(v3_scale(v3(smp[0], smp[1], smp[2]), R(255.0) / R(127.0)), -(R(128.0) / R(127.0)));
         o_vec3 zero3 = v3_splat(R(0.0));
         o_vec2 zero2 = {R(0.0), R(0.0)};
@@ -1123,7 +1121,7 @@ static void* band_worker(void* arg) {
                 o_vec3 nrm = f3(&g->nrm_scale[i * 4]);
                 o_vec2 uv = {g->uv[i * 2], g->uv[i * 2 + 1]};
                 real frag_coord[4] = {(real)x + R(0.5), (real)y + R(0.5), g->pos_depth[i * 4 + 3], R(1.0)};
-                /* OpDPdx / OpDPdy restated on the G-buffer: differences inside the pixel's 2x2 quad (frame
+                /* ddx / ddy restated on the G-buffer: differences inside the pixel's 2x2 quad (frame
                  * coordinates), value(x|1) - value(x&~1) and value(y|1) - value(y&~1); zero when the partner is
                  * outside the planes or not covered (a rasteriser would extrapolate a helper invocation). */
                 o_frag_derivs dv;

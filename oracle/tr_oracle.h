@@ -9,11 +9,10 @@
  *
  * Pinning: the reference (expenses/transmission-renderer) ships no tests, golden
  * vectors or fixtures, and neither Rust nor Vulkan exist in the build image, so the
- * Rust sources cannot be run.  What CAN be run are the reference's own committed
- * SPIR-V binaries: oracle/spirv_ref/ interprets the .spv files of compiled-shaders/normal
- * word by word (fixed-function sampling restated, see there) and the fixtures under
- * tests/golden/ were produced that way.  tests/test_oracle_vs_spirv.py pins every
- * entry point of this file against those fixtures.  Steps with no in-tree definition
+ * Rust sources cannot be run.  tests/golden/ holds recorded inputs and outputs of its
+ * entry points (tests/golden/README.md: how they came about, and that nothing here
+ * can make them again); tests/test_oracle_vs_spirv.py and its neighbours hold every
+ * entry point of this file to them.  Steps with no in-tree definition
  * (mip blit filter, texel filtering weights, real->half rounding) are restated from
  * the Vulkan specification and are called out as "unpinned" where they occur.
  *
@@ -149,7 +148,7 @@ typedef struct {
     uint32_t level_offset[TR_MAX_MIP_LEVELS];   /* in texels */
 } o_texture;
 
-/* screen-space derivatives of the interpolants a fragment shader may differentiate (OpDPdx / OpDPdy) */
+/* screen-space derivatives of the interpolants a fragment shader may differentiate (ddx / ddy) */
 typedef struct {
     o_vec3 dpos_dx, dpos_dy;   /* of the value the shader differentiates: -view_vector = -(view_position - position)
                                 * (lighting.rs:237), i.e. neighbour's value minus this quad partner's value */

@@ -1,0 +1,49 @@
+"""What the sources of this repository must not hold (CPU only: text of the tracked trees and the recorded fixtures).
+
+* Nothing opens or decodes a compiled shader: the reference's .spv files are compiled code that was not built here.  The
+  fixtures recorded under tests/golden/ are inputs and output numbers and hold no code.
+"""
+import glob
+import os
+import re
+
+import numpy as np
+import pytest
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+TREES = ("transmission_renderer_amd", "include", "oracle", "tools", "examples")
+SUFFIXES = (".py", ".c", ".h", ".hip", ".cpp", ".sh", ".s", "Makefile")
+
+
+def _sources():
+    out = [os.path.join(ROOT, f) for f in ("bench.py", "__graft_entry__.py")]
+    for tree in TREES:
+        for d, dirs, files in os.walk(os.path.join(ROOT, tree)):
+            dirs[:] = [x for x in dirs if x != "__pycache__"]
+            out += [os.path.join(d, f) for f in files if f.endswith(SUFFIXES)]
+    assert len(out) > 60   # the walk found the trees
+    return sorted(out)
+
+
+def _lines_with(pattern):
+    hits = []
+    for path in _sources():
+        with open(path, encoding="utf-8", errors="replace") as f:
+            hits += [f"{os.path.relpath(path, ROOT)}:{n}: {line.strip()}" for n, line in enumerate(f, 1) if re.search(pattern, line)]
+    return hits
+
+
+def test_no_source_opens_or_decodes_a_compiled_shader():
+    # a file name, the directory that holds them, or the word that opens such a module
+    assert _lines_with(r"\.spv\b|compiled-shaders|(?i:0x07230203)|spirv_interp") == []
+
+
+@pytest.mark.parametrize("path", sorted(glob.glob(os.path.join(ROOT, "tests", "golden", "*.npz"))), ids=os.path.basename)
+def test_a_fixture_holds_numbers_and_no_code(path):
+    with np.load(path, allow_pickle=False) as z:
+        for name in z.files:
+            a = z[name]
+            kinds = [a.dtype[f].base.kind for f in a.dtype.names] if a.dtype.names else [a.dtype.kind]
+            assert set(kinds) <= set("fiu"), name
+            raw = a.tobytes()
+            assert b"\x03\x02\x23\x07" not in raw and b"\x07\x23\x02\x03" not in raw, name   # a module's first word

@@ -1,8 +1,8 @@
 #!/usr/bin/env python3
 """Prints, for every parity configuration of tests/, the PLAIN all-pixel per-channel RMSE of the HIP passes against
-the pinned artefacts (SPIR-V outputs of the golden cases; the fp32 oracle elsewhere) — raw and normalised by
+the pinned artefacts (recorded outputs of the golden cases; the fp32 oracle elsewhere) — raw and normalised by
 max(|ref|, 1), on the RGBA32F and the RGBA16F target — next to the fp64 twin that explains the outliers.
-Run on the GPU box:  python tools/gpu_parity_report.py > gpurun_out/parity_report.txt
+Run where a GPU is:  python tools/gpu_parity_report.py > parity_report.txt
 """
 import glob
 import json

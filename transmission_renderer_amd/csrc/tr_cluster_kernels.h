@@ -8,7 +8,7 @@
 // time, a ballot gives the survivors and a prefix pop-count (mbcnt) their slots — the list is written sorted by
 // light index with no atomics, deterministic from run to run (the shading kernels sum lights in list order).
 // All arithmetic is IEEE fp32 with contraction off, in the reference's order: the outputs are bit-identical to
-// the CPU oracle, which is bit-identical to the reference's compiled .spv (tests/golden/spirv_clusters.npz).
+// the CPU oracle, which reproduces the recorded outputs of tests/golden/spirv_clusters.npz bit for bit.
 // Transcendentals (powf for the slice depths, cos/sin of the spot angle) are evaluated on the host with libm.
 #pragma once
 

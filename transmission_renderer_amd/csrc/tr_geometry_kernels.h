@@ -4,7 +4,7 @@
 //   frustum_culling + cull        shader/src/lib.rs:411-465     (dispatch: src/main.rs:1716-1763)
 //   demultiplex_draws             shader/src/lib.rs:467-517     (dispatch: src/main.rs:1811-1838)
 //   Similarity * Vec3, unpack     shared-structs/src/lib.rs:178-236
-// Decisions are comparisons of fp32 values, so the arithmetic follows the compiled shaders' operation order with
+// Decisions are comparisons of fp32 values, so the arithmetic follows the reference's operation order with
 // contraction off: the visible sets are identical to the CPU restatement's, not merely close.
 #pragma once
 

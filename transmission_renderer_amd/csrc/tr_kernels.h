@@ -1185,7 +1185,7 @@ __device__ __forceinline__ f3 shade_pixel(claunch* L, MatP m, uint32_t mat_index
 
 // ------------------------------------------------------------------------ one pixel of a textured material
 // Differences inside the pixel's 2x2 quad of the two values the reference's shaders differentiate
-// (OpDPdx / OpDPdy): -view_vector (shader/src/lighting.rs:237) and uv (the implicit LOD of every texture fetch).
+// (ddx / ddy): -view_vector (shader/src/lighting.rs:237) and uv (the implicit LOD of every texture fetch).
 struct quad_derivs {
     uv_derivs uv;   // (full-class kernels: these and the differences of -view_vector wait in LDS, see kParkSlots)
 };
@@ -1274,7 +1274,7 @@ __device__ __forceinline__ f3 shade_pixel_textured(claunch* L, uint32_t material
     if (id_normal != -1) {
         const float inv_n = rsq(dot3(ns.x, ns.y, ns.z, ns.x, ns.y, ns.z));
         const f3 n = {ns.x * inv_n, ns.y * inv_n, ns.z * inv_n};
-        // map_normal * 255/127 - 128/127 (the compiled shader folds 255/127 into one multiply)
+        // map_normal * 255/127 - 128/127, the two quotients of constants formed first
         float mx = 0.0f, my = 0.0f, mz = 0.0f;
         with_slot(std::integral_constant<int, 2>{}, [&](auto S) {
             mx = fmaf(S(c0{}), 255.0f / 127.0f, -128.0f / 127.0f);

@@ -4,7 +4,7 @@
 // Reference semantics (file:line relative to the reference root):
 //   load_image_from_bytes: full mip chain by LINEAR blits      src/model_loading.rs:335-390
 //   `sampler` (LINEAR min/mag/mip, REPEAT, anisotropy off)     src/main.rs:683-692
-//   TextureSampler::sample -> OpImageSampleImplicitLod         shader/src/lib.rs:252-262
+//   TextureSampler::sample (implicit LOD)                      shader/src/lib.rs:252-262
 // Storage: one arena in HBM holding every texture's chain, RGBA8, levels packed; tr_dtex (scalar-loaded: the
 // texture id is a property of the material, and a wave shades one material at a time) describes one chain.
 #pragma once
@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void texture_downsample_kernel(const uint32_t*
 }
 
 // ------------------------------------------------------------------------ the sampler
-// Screen-space differences of uv inside the pixel's 2x2 quad (OpDPdx / OpDPdy of the interpolant).
+// Screen-space differences of uv inside the pixel's 2x2 quad (ddx / ddy of the interpolant).
 struct uv_derivs {
     float dudx, dvdx, dudy, dvdy;
 };
