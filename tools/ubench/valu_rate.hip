@@ -3,17 +3,13 @@
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
-typedef float v2f __attribute__((ext_vector_type(2)));
 #define N_ITER 4096
 template <int KIND>
 __global__ __launch_bounds__(256) void k(float* out, float a, float b) {
     float x0 = threadIdx.x * 1e-3f, x1 = x0 + 1, x2 = x0 + 2, x3 = x0 + 3, x4 = x0 + 4, x5 = x0 + 5, x6 = x0 + 6, x7 = x0 + 7;
-    v2f p0 = {x0, x1}, p1 = {x2, x3}, p2 = {x4, x5}, p3 = {x6, x7}, pa = {a, a}, pb = {b, b};
     for (int i = 0; i < N_ITER; ++i) {
         if (KIND == 0) { x0 = __builtin_fmaf(x0, a, b); x1 = __builtin_fmaf(x1, a, b); x2 = __builtin_fmaf(x2, a, b); x3 = __builtin_fmaf(x3, a, b);
                          x4 = __builtin_fmaf(x4, a, b); x5 = __builtin_fmaf(x5, a, b); x6 = __builtin_fmaf(x6, a, b); x7 = __builtin_fmaf(x7, a, b); }
-        if (KIND == 1) { p0 = __builtin_elementwise_fma(p0, pa, pb); p1 = __builtin_elementwise_fma(p1, pa, pb); p2 = __builtin_elementwise_fma(p2, pa, pb); p3 = __builtin_elementwise_fma(p3, pa, pb);
-                         p0 = __builtin_elementwise_fma(p0, pb, pa); p1 = __builtin_elementwise_fma(p1, pb, pa); p2 = __builtin_elementwise_fma(p2, pb, pa); p3 = __builtin_elementwise_fma(p3, pb, pa); }
         if (KIND == 2) { x0 = __builtin_amdgcn_rcpf(x0); x1 = __builtin_amdgcn_rcpf(x1); x2 = __builtin_amdgcn_rcpf(x2); x3 = __builtin_amdgcn_rcpf(x3);
                          x4 = __builtin_amdgcn_rcpf(x4); x5 = __builtin_amdgcn_rcpf(x5); x6 = __builtin_amdgcn_rcpf(x6); x7 = __builtin_amdgcn_rcpf(x7); }
         if (KIND == 3) { x0 = fmaxf(x0, a) ; x1 = fminf(x1, b); x2 = fmaxf(x2, a); x3 = fminf(x3, b); x4 = fmaxf(x4, b); x5 = fminf(x5, a); x6 = fmaxf(x6, b); x7 = fminf(x7, a);
@@ -58,7 +54,7 @@ __global__ __launch_bounds__(256) void k(float* out, float a, float b) {
         if (KIND == 23) { asm volatile("v_max3_f32 %0, %0, %1, %2\n v_max3_f32 %1, %1, %2, %3\n v_floor_f32 %2, %2\n v_floor_f32 %3, %3\n v_cvt_u32_f32 %4, %4\n v_cvt_f32_u32 %5, %5\n v_cvt_pk_f16_f32 %6, %6, %7\n v_cvt_f32_ubyte0 %7, %7"
                                       : "+v"(x0), "+v"(x1), "+v"(x2), "+v"(x3), "+v"(x4), "+v"(x5), "+v"(x6), "+v"(x7)); }
     }
-    out[blockIdx.x * 256 + threadIdx.x] = x0 + x1 + x2 + x3 + x4 + x5 + x6 + x7 + p0.x + p0.y + p1.x + p1.y + p2.x + p2.y + p3.x + p3.y;
+    out[blockIdx.x * 256 + threadIdx.x] = x0 + x1 + x2 + x3 + x4 + x5 + x6 + x7;
 }
 template <int KIND> void run(const char* name, int blocks, float* d) {
     hipEvent_t e0, e1; hipEventCreate(&e0); hipEventCreate(&e1);
@@ -74,7 +70,7 @@ template <int KIND> void run(const char* name, int blocks, float* d) {
 int main() {
     float* d; hipMalloc(&d, 8192 * 256 * 4);
     for (int blocks : {8192}) {
-        run<0>("v_fma_f32", blocks, d); run<1>("v_pk_fma_f32", blocks, d); run<4>("v_mul/add_f32", blocks, d); run<3>("v_max/min_f32", blocks, d);
+        run<0>("v_fma_f32", blocks, d); run<4>("v_mul/add_f32", blocks, d); run<3>("v_max/min_f32", blocks, d);
         run<14>("v_fma_f32 (3 vgpr srcs)", blocks, d); run<15>("v_mul/fmac/add 2-src vgpr", blocks, d); run<13>("fma/mul with sgpr/literal", blocks, d);
         run<8>("v_mov_b32", blocks, d); run<9>("v_sub/max/min_f32", blocks, d); run<10>("v_cmp+v_cndmask", blocks, d); run<11>("v_fma_mix_f32", blocks, d); run<12>("int add/shift/and/mul24", blocks, d);
         run<16>("v_fma_f32 sgpr src", blocks, d); run<17>("VOP2 mul/add/sub/max sgpr src0", blocks, d); run<18>("VOP2 with 32-bit literal", blocks, d);

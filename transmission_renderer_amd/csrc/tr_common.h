@@ -16,7 +16,7 @@ constexpr float kPi = 3.14159265358979323846f;
 constexpr float kFrac1Pi = 0.318309886183790671538f;
 constexpr float kLog2e = 1.44269504088896340736f;
 
-typedef float v2f __attribute__((ext_vector_type(2)));  // one v_pk_*_f32 operand
+typedef float v2f __attribute__((ext_vector_type(2)));  // a pair of like terms; two scalar instructions each (packed fp32 is off)
 
 // Tables that a whole wave reads at one address (material, lights, cluster lists, level geometry)
 // are addressed through the constant address space: a uniform load from it is always issued on the

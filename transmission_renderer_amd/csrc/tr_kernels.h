@@ -22,8 +22,8 @@
 //     (the last form keeps d_ggx well conditioned at low roughness); the mirrored light of
 //     transmission_btdf needs no vector at all (n.l' = -n.l, v.l' = v.l - 2 n.l n.v, and
 //     n x (v+l') = n x (v+l)), so the two lobes share the vector work;  D*V is one reciprocal per lobe,
-//     x^5 three multiplies.  (On gfx950 v_pk_fma_f32 issues at half the rate of v_fma_f32 — tools/ubench —
-//     so packing buys nothing: the build disables packed-fp32 selection.)
+//     x^5 three multiplies.  (On gfx950 v_pk_fma_f32 issues at half the rate of v_fma_f32, and some packed forms have given wrong results:
+//     the build disables packed-fp32 selection.)
 //   * horizontally adjacent texels come in one 16-byte load, filtered as one weighted sum of v_fma_mix_f32;
 //   * the cluster x / y lookups are exact tables (built with the reference's own IEEE division on the host); the
 //     depth slice is one v_log_f32 made exact against a table of slice thresholds (depth_slice);
