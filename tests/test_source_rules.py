@@ -5,15 +5,18 @@
 * No source, script or test names an instruction that writes through the scalar data cache (scalar stores and atomics, the
   cache's write-back and discard), comments included: machines that refuse such code refuse the whole tree for it.  This
   file has to name them, and is therefore kept off such machines (.gpurunignore); none of its tests needs a GPU.
-* No kernel is written with packed fp32 instructions: some of their forms have given wrong results on MI355X, rarely and
-  without an error.
+* No kernel is written with packed fp32 instructions, and none is compiled to them: some of their forms have given wrong
+  results on MI355X, rarely and without an error.  hipcc -O3 makes them by itself unless told not to.
 """
 import glob
 import os
 import re
+import subprocess
 
 import numpy as np
 import pytest
+
+from test_kernel_resources import _code_object
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 TREES = ("transmission_renderer_amd", "include", "oracle", "tools", "examples")
@@ -64,3 +67,27 @@ def test_no_source_names_a_write_through_the_scalar_data_cache():
 def test_no_kernel_is_written_with_packed_fp32_instructions():
     # in a string: an asm statement, or the name that a benchmark prints for one.  Prose about them is no instruction
     assert _lines_with(r"\"[^\"]*\bv_pk_(?:add|mul|fma)_f32") == []
+
+
+@pytest.mark.parametrize("name", ["libtr_shade.so", "pattern_ceiling"])
+def test_no_built_kernel_holds_packed_fp32_instructions(name, tmp_path):
+    objdump = "/opt/rocm/lib/llvm/bin/llvm-objdump"
+    path = os.path.join(ROOT, "transmission_renderer_amd", name)
+    if not os.path.exists(path):
+        pytest.fail(f"{path} is missing: run __graft_entry__.build() first")
+    if not os.path.exists(objdump):
+        pytest.skip("llvm-objdump not available")
+    co = tmp_path / "gfx950.co"
+    co.write_bytes(_code_object(path))
+    asm = subprocess.run([objdump, "-d", str(co)], capture_output=True, text=True, check=True).stdout
+    assert "s_endpgm" in asm
+    assert sorted(set(re.findall(r"\bv_pk_(?:add|mul|fma)_f32", asm))) == []
+
+
+def test_every_hipcc_command_turns_packed_fp32_off():
+    # the flag lists that build() and tools/ compile with, and the commands that comments give
+    commands = _lines_with(r"--offload-arch=gfx950 -|\"--offload-arch=gfx950\"")
+    assert len(commands) >= 9
+    assert [c for c in commands if "-packed-fp32-ops" not in c and "NO_PACKED_FP32" not in c] == []
+    import __graft_entry__ as g
+    assert g.NO_PACKED_FP32 == ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]

@@ -4,7 +4,7 @@
 // XCD only.  Every lane one atomicMax on its own word of a 3840x2160 buffer, 8x8 pixel blocks, `passes` passes (so words
 // are hit repeatedly), blocks dealt (a) round-robin over all waves, (b) by XCD: the workgroup on XCD x (hardware places
 // workgroup b on XCD b % 8) takes blocks of row band x only.  The final buffer is checked against the expected maxima.
-// hipcc --offload-arch=gfx950 -O2 atomic_scope.hip -o atomic_scope && ./atomic_scope
+// hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops atomic_scope.hip -o atomic_scope && ./atomic_scope
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // Does a wave64 VALU instruction cost less on gfx950 when half of its lanes are switched off?  (SIMD-32: a wave64
-// instruction issues over two passes of 32 lanes.)  Build: hipcc --offload-arch=gfx950 -O3 exec_mask.hip -o exec_mask
+// instruction issues over two passes of 32 lanes.)  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops exec_mask.hip -o exec_mask
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #define N_ITER 4096

@@ -1,7 +1,7 @@
 // Do atomics on DIFFERENT words of one 128-byte line queue up like atomics on one word?  8 192 waves take 16 tickets each from
 // one of 32 counters (lane 0, atomic with return, the wave waits for each), the counters `stride` words apart: 1 = all 32 in
 // one line, 32 = a line each, 64 = a line each with a line between.  One counter for reference.
-//   hipcc --offload-arch=gfx950 -O2 tools/ubench/line_atomics.hip -o /tmp/line_atomics && /tmp/line_atomics
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench/line_atomics.hip -o /tmp/line_atomics && /tmp/line_atomics
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

@@ -12,7 +12,7 @@
 // — the number the memory side sustains per CU for THIS pattern.  The last rows repeat the 8-wave measurement with a block
 // of N dependent fma per pixel between the wait and the store (the arithmetic a real pass must overlap with the stream).
 //
-// Build + run:  hipcc --offload-arch=gfx950 -O3 tools/ubench/pattern_ceiling.hip -o /tmp/pattern_ceiling && /tmp/pattern_ceiling
+// Build + run:  hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench/pattern_ceiling.hip -o /tmp/pattern_ceiling && /tmp/pattern_ceiling
 #include <hip/hip_runtime.h>
 #include <cstdint>
 #include <cstdio>

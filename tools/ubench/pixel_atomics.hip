@@ -1,6 +1,6 @@
 // Throughput of the rasteriser's per-pixel visibility update on gfx950: every lane one 64-bit atomicMax on its own word,
 // a wave covering an 8x8 pixel block of a 3840-wide buffer (8 rows x 64 B), against plain 8-byte stores and 32-bit
-// atomics of the same shape.   hipcc --offload-arch=gfx950 -O2 pixel_atomics.hip -o pixel_atomics && ./pixel_atomics
+// atomics of the same shape.   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops pixel_atomics.hip -o pixel_atomics && ./pixel_atomics
 #include <hip/hip_runtime.h>
 #include <cstdio>
 

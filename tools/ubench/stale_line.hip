@@ -7,7 +7,7 @@
 //            control: its bytes stay in the writer's L2), waits for the stores, signals
 //   stage 3: the stage-1 workgroup itself (same CU: L1 + L2) and workgroup r + 8 (same XCD, another CU or not: L2) read word 16
 //            with a plain load.  Stale = the value from before stage 2.
-//   hipcc --offload-arch=gfx950 -O2 tools/ubench/stale_line.hip -o /tmp/stale_line && /tmp/stale_line
+//   hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench/stale_line.hip -o /tmp/stale_line && /tmp/stale_line
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <cstdlib>

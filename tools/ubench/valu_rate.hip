@@ -1,5 +1,5 @@
 // VALU issue-rate microbenchmark for gfx950: wave64 instructions per cycle per SIMD for the instruction
-// classes the shading kernel is made of.  Build: hipcc --offload-arch=gfx950 -O3 valu_rate.hip -o valu_rate
+// classes the shading kernel is made of.  Build: hipcc --offload-arch=gfx950 -O3 -Xclang -target-feature -Xclang -packed-fp32-ops valu_rate.hip -o valu_rate
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>

@@ -1,5 +1,5 @@
 // Which SIMD do the four waves of a 256-thread workgroup land on?  (HW_ID bits 5:4 = SIMD, 11:8 = CU, 15:13 = SE on gfx9.)
-// hipcc --offload-arch=gfx950 -O2 tools/ubench/wave_simd.hip -o /tmp/wave_simd && /tmp/wave_simd
+// hipcc --offload-arch=gfx950 -O2 -Xclang -target-feature -Xclang -packed-fp32-ops tools/ubench/wave_simd.hip -o /tmp/wave_simd && /tmp/wave_simd
 #include <hip/hip_runtime.h>
 #include <cstdio>
 #include <vector>
