@@ -4,7 +4,7 @@
   fixtures recorded under tests/golden/ are inputs and output numbers and hold no code.
 * No source, script or test names an instruction that writes through the scalar data cache (scalar stores and atomics, the
   cache's write-back and discard), comments included: machines that refuse such code refuse the whole tree for it.  This
-  file has to name them, and is therefore kept off such machines (.gpurunignore); none of its tests needs a GPU.
+  file has to name them, and is therefore left out of what is sent to such machines; none of its tests needs a GPU.
 * No kernel is written with packed fp32 instructions, and none is compiled to them: some of their forms have given wrong
   results on MI355X, rarely and without an error.  hipcc -O3 makes them by itself unless told not to.
 """
